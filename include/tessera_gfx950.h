@@ -401,7 +401,7 @@ int tessera_gfx950_flash_attn_gqa_bf16_dev(const void* Q, const void* K, const v
  * bounds and score transform of its CPU kernel (avx512_flash_attn_f32.cpp:115-196):
  * window > 0 keeps, per query row i, the `window` keys ending at the causal diagonal
  * i + max(Sk - Sq, 0) (causal != 0) or window/2 keys either side of it (causal == 0);
- * softcap > 0 passes each scaled score through cap * tanh(s / cap) before the
+ * softcap > 0 (infinity: none) passes each scaled score through cap * tanh(s / cap) before the
  * softmax.  0 disables either.  A row with no visible key gives O = 0, LSE = -inf. */
 int tessera_gfx950_flash_attn_ext_f16(const void* Q, const void* K, const void* V, void* O, void* LSE,
                                       int B, int Hq, int Hkv, int Sq, int Sk, int D, float scale,

@@ -18,10 +18,10 @@ bool bad_attn(int B, int Hq, int Hkv, int Sq, int Sk, int D) {
   return false;
 }
 
-template <class T, int DP, bool EXT, bool PAD, int W>
+template <class T, int DP, bool EXT, bool PAD, int W, bool FAR = false>
 int launch_flash_as(const FlashParams& p, int nsplit, hipStream_t s) {
   using G = FlashGeom<DP, W>;
-  auto kern = flash_fwd_kernel<T, DP, EXT, PAD, W>;
+  auto kern = flash_fwd_kernel<T, DP, EXT, PAD, W, FAR>;
   static std::once_flag once;
   static hipError_t attr_err = hipSuccess;
   std::call_once(once, [&] {
@@ -77,7 +77,10 @@ int launch_flash(const FlashParams& p, hipStream_t s) {
     }
     return launch_flash_as<T, DP, EXT, PAD, 8>(p, f.nsplit, s);
   } else {
-    return launch_flash_as<T, DP, EXT, PAD, 8>(p, split8(problem, FlashGeom<DP>::BQ), s);
+    const int nsplit = split8(problem, FlashGeom<DP>::BQ);
+    // (caps over kPlainCap: one kernel for a whole and for a padded head dimension)
+    if (EXT && p.softcap > kPlainCap) return launch_flash_as<T, DP, true, true, 8, true>(p, nsplit, s);
+    return launch_flash_as<T, DP, EXT, PAD, 8>(p, nsplit, s);
   }
 }
 
@@ -202,7 +205,7 @@ int flash_dev(const void* Q, const void* K, const void* V, void* O, void* LSE, i
   p.causal = causal ? 1 : 0;
   p.out_storage = out_storage ? 1 : 0;
   p.window = window;
-  p.softcap = softcap;
+  p.softcap = std::isinf(softcap) ? 0.f : softcap;       // (cap tanh(s / cap) is s itself in the limit)
   p.bias = bias;
   // 16-byte accesses: pointers and strides must be multiples of 16 bytes (8 elements of the
   // 16-bit operands; O in f32 is then aligned as well).

@@ -55,16 +55,19 @@ __host__ __device__ inline bool folds(const PagedParams& p) { return p.scale > 1
 // multiplier 2 cap log2(e) goes into the exponential's FMA and whose constant only the LSE needs (base).  B 4, 2048 tokens on
 // 3000 keys, cap 30: 457 us with those two FMAs in the walk, 433 without; and 357 with the choice between cap and plain scale made once a
 // tile, not at each score (296 without a cap).  A cap under 1e-8 is one of 1e-8, no score being off by
-// more than that: the mask's sentinel times the slope has to stay far below every score.
+// more than that: the mask's sentinel times the slope has to stay far below every score.  Caps over kPlainCap (far): the walk carries the
+// exponent itself, from far_exponent.
 struct SoftCap {
-  float in = 0.f, slope = 1.0f, base = 0.f;
+  float in = 0.f, top = 0.f, slope = 1.0f, base = 0.f;
   __device__ __forceinline__ SoftCap() {}
-  __device__ __forceinline__ explicit SoftCap(const PagedParams& p) {
+  __device__ __forceinline__ SoftCap(const PagedParams& p, bool far) {
     if (!(p.softcap > 0.f)) return;
-    const float cap2 = 1.44269504088896340736f * fmaxf(p.softcap, 1e-8f);
-    in = 2.0f * 1.44269504088896340736f * p.scale / fmaxf(p.softcap, 1e-8f);
-    slope = 2.0f * cap2;
-    base = cap2;
+    const float cap = far ? fminf(p.softcap, 2.0e38f) : fmaxf(p.softcap, 1e-8f);
+    in = 2.0f * 1.44269504088896340736f * p.scale / cap;
+    top = 1.44269504088896340736f * cap;
+    if (far) return;
+    slope = 2.0f * top;
+    base = top;
   }
   __device__ __forceinline__ float form(float s) const { return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s * in)); }
 };

@@ -170,7 +170,8 @@ __device__ __forceinline__ void store_o4(const PagedParams& p, int token, int hq
   else *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.O) + at) = v;
 }
 
-template <class T, int FMT, int DP, int NQ>
+// FAR: a soft cap over kPlainCap.
+template <class T, int FMT, int DP, int NQ, bool FAR>
 __global__ __launch_bounds__((FewGeom<FMT, DP>::THREADS), (DP <= 128 && NQ == 1 ? 2 : 1)) void paged_few_kernel(const PagedFewParams fp) {
   using G = FewGeom<FMT, DP>;
   using TV = typename std::conditional<FMT == kStorage, T, F16>::type;    // type of the second product
@@ -363,7 +364,7 @@ __global__ __launch_bounds__((FewGeom<FMT, DP>::THREADS), (DP <= 128 && NQ == 1 
   // A score's exponent in base 2 is scale log2(e) s, folded into the exponential or applied before it.
   const float c = p.scale * 1.44269504088896340736f;
   const bool fold = folds(p);
-  const SoftCap cap = fold ? SoftCap() : SoftCap(p);
+  const SoftCap cap = fold ? SoftCap() : SoftCap(p, FAR);
   const float slope = fold || !(p.softcap > 0.f) ? c : cap.slope;
   const float cs = CODES ? 1.0f : fold ? c : cap.slope;  // what is left to multiply at the exponential
 
@@ -438,7 +439,10 @@ __global__ __launch_bounds__((FewGeom<FMT, DP>::THREADS), (DP <= 128 && NQ == 1 
 #pragma unroll
     for (int qt = 0; qt < NQ; ++qt) {
       if (!fold) {
-        if (p.softcap > 0.f) {
+        if constexpr (FAR) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sc[qt][r] = far_exponent(sc[qt][r], c, cap.in, cap.top);
+        } else if (p.softcap > 0.f) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) sc[qt][r] = cap.form(sc[qt][r]);
         } else if (!CODES) {

@@ -39,26 +39,31 @@ struct FewKernel {
   void (*run)(const PagedFewParams);
   int threads, lds, per_cu;
 };
-template <class T, int FMT, int DP, int NQ>
-FewKernel few_kernel() {
+template <class T, int FMT, int DP, int NQ, bool FAR>
+FewKernel few_kernel_as() {
   using G = FewGeom<FMT, DP>;
   static std::once_flag once;
   static int per_cu = 0;
   std::call_once(once, [] {
-    const void* kern = reinterpret_cast<const void*>(paged_few_kernel<T, FMT, DP, NQ>);
+    const void* kern = reinterpret_cast<const void*>(paged_few_kernel<T, FMT, DP, NQ, FAR>);
     if (lds_limit(kern, G::SMEM) != kOk || hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kern, G::THREADS, G::SMEM) != hipSuccess)
       per_cu = 0;
   });
-  return FewKernel{paged_few_kernel<T, FMT, DP, NQ>, G::THREADS, G::SMEM, per_cu};
+  return FewKernel{paged_few_kernel<T, FMT, DP, NQ, FAR>, G::THREADS, G::SMEM, per_cu};
+}
+template <class T, int FMT, int DP, int NQ>
+FewKernel few_kernel(const PagedParams& p) {
+  return p.softcap > kPlainCap ? few_kernel_as<T, FMT, DP, NQ, true>() : few_kernel_as<T, FMT, DP, NQ, false>();
 }
 template <class T, int FMT>
-FewKernel few_kernel_for(int D, int rows) {
-  if (D <= 64) return rows <= 32 ? few_kernel<T, FMT, 64, 1>() : rows <= 64 ? few_kernel<T, FMT, 64, 2>() : few_kernel<T, FMT, 64, 4>();
-  if (D <= 128) return rows <= 32 ? few_kernel<T, FMT, 128, 1>() : few_kernel<T, FMT, 128, 2>();
-  return few_kernel<T, FMT, 256, 1>();
+FewKernel few_kernel_for(const PagedParams& p, int rows) {
+  const int D = p.c.D;
+  if (D <= 64) return rows <= 32 ? few_kernel<T, FMT, 64, 1>(p) : rows <= 64 ? few_kernel<T, FMT, 64, 2>(p) : few_kernel<T, FMT, 64, 4>(p);
+  if (D <= 128) return rows <= 32 ? few_kernel<T, FMT, 128, 1>(p) : few_kernel<T, FMT, 128, 2>(p);
+  return few_kernel<T, FMT, 256, 1>(p);
 }
 
-template <class T, int FMT, int DP, int W, bool EXT>
+template <class T, int FMT, int DP, int W, int EXT>
 int launch_tile_as(const PagedTileParams& tp, int blocks, hipStream_t s) {
   constexpr int SMEM = TileGeom<DP, W>::SMEM(FMT != kStorage);
   auto kern = paged_tile_kernel<T, FMT, DP, W, EXT>;
@@ -71,7 +76,8 @@ int launch_tile_as(const PagedTileParams& tp, int blocks, hipStream_t s) {
 }
 template <class T, int FMT, int DP, int W>
 int launch_tile(const PagedTileParams& tp, int blocks, hipStream_t s) {
-  return folds(tp.p) ? launch_tile_as<T, FMT, DP, W, false>(tp, blocks, s) : launch_tile_as<T, FMT, DP, W, true>(tp, blocks, s);
+  if (folds(tp.p)) return launch_tile_as<T, FMT, DP, W, 0>(tp, blocks, s);
+  return tp.p.softcap > kPlainCap ? launch_tile_as<T, FMT, DP, W, 2>(tp, blocks, s) : launch_tile_as<T, FMT, DP, W, 1>(tp, blocks, s);
 }
 template <class T, int FMT>
 int launch_tile_for(const PagedTileParams& tp, const PagedPlan& plan, hipStream_t s) {
@@ -165,7 +171,7 @@ int launch_paged(const PagedParams& p, hipStream_t s) {
   tp.min_rows = plan.few_rows;
   FewKernel few{};
   if (plan.few) {
-    few = few_kernel_for<T, FMT>(p.c.D, plan.few_rows);
+    few = few_kernel_for<T, FMT>(p, plan.few_rows);
     if (few.per_cu <= 0) return kDeviceFailed;
     // As many equal shares as the chip holds workgroups for every head, at least one for a sequence and two tiles
     // for a wave.  Starting a sequence costs about two steps of a workgroup.

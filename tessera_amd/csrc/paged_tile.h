@@ -105,9 +105,9 @@ __device__ __forceinline__ bool find_block(const PagedTileParams& tp, int index,
   return false;
 }
 
-// EXT: a soft cap, or a scale that is not well above zero: scores become exponents before the mask; else the scale is folded into
-// the exponential.
-template <class T, int FMT, int DP, int W, bool EXT>
+// EXT 0: the scale is folded into the exponential.  1: a soft cap, or a scale that is not well above zero: scores become exponents
+// before the mask.  2: the same for a cap over kPlainCap.
+template <class T, int FMT, int DP, int W, int EXT>
 __global__ __launch_bounds__((TileGeom<DP, W>::THREADS), (DP > 128 ? 1 : 2)) void paged_tile_kernel(const PagedTileParams tp) {
   using G = TileGeom<DP, W>;
   using TV = typename std::conditional<FMT == kStorage, T, BF16>::type;
@@ -286,7 +286,7 @@ __global__ __launch_bounds__((TileGeom<DP, W>::THREADS), (DP > 128 ? 1 : 2)) voi
 #pragma unroll
     for (int r = 0; r < 16; ++r) o_acc[dt][r] = 0.f;
   const float c = p.scale * 1.44269504088896340736f;
-  const SoftCap cap = EXT ? SoftCap(p) : SoftCap();
+  const SoftCap cap = EXT ? SoftCap(p, EXT == 2) : SoftCap();
   const float cs = EXT ? cap.slope : c;                  // see folds()
 
   // ---- LDS read addresses: of step ks k_rd ^ 32 ks, of output columns 32 dt .. v_rd ^ 64 dt (chunk numbers are swizzled by
@@ -362,8 +362,13 @@ __global__ __launch_bounds__((TileGeom<DP, W>::THREADS), (DP > 128 ? 1 : 2)) voi
           sc[kt][4 * a + 0] *= x.x; sc[kt][4 * a + 1] *= x.y; sc[kt][4 * a + 2] *= x.z; sc[kt][4 * a + 3] *= x.w;
         }
     }
-    if constexpr (EXT) {
-      if (p.softcap > 0.f) {
+    if constexpr (EXT != 0) {
+      if constexpr (EXT == 2) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sc[kt][r] = far_exponent(sc[kt][r], c, cap.in, cap.top);
+      } else if (p.softcap > 0.f) {
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
