@@ -468,7 +468,8 @@ int tessera_gfx950_flash_attn_bias_bf16_dev(const void* Q, const void* K, const 
  * format 0: the 16-bit storage type of the calls.  1: int8 codes, 2: e4m3fn codes; value = code * scale with one f32 scale
  * for each (page, place, head) of K and of V, and for a row x
  *     scale = max(max|x| * (1 / top), 1e-12),  code = round-to-nearest-even(clip(x / scale, +-top)),  top = 127 | 448
- * in f32 (attention over a cache of another writer: scales are positive; one under 1e-30 may count as 1e-30): 1 / top is the nearest f32, x / scale the correctly rounded quotient.  A row with an infinity or a NaN reads back as nothing finite.
+ * in f32 (attention over a cache of another writer: scales are positive; one under 1e-25 may count as 1e-25): 1 / top is the nearest f32,
+ * x / scale the correctly rounded quotient.  A row with an infinity or a NaN reads back as nothing finite.
  *
  * Strides are element strides of (page, place, head), the last dimension is contiguous; [pages, page_size, heads, D] and
  * [pages, heads, page_size, D] are both served.  K, V and their strides lie on the 16-byte grid; a stride is under 2 GiB
@@ -517,7 +518,7 @@ int tessera_gfx950_kv_cache_read_bf16_dev(const tessera_gfx950_kv_cache* cache, 
  *
  * Scores, softmax statistics and sums are f32.  A probability is rounded once before the second product, to the storage type; over
  * 8-bit formats the second product's weights, probability times scale, have 11 bits where a sequence has few rows, else 8, and 16 in
- * f16 programs.  Keys that a token does not see
+ * f16 programs.  Weights of 11 bits (f16) keep them down to 2^-28 of a row's largest and are nothing under 2^-39 of it.  Keys that a token does not see
  * leave its row as it is whatever they hold, infinities and NaN among it.  How a sequence's keys are divided, and so the order of
  * the sums, depends on the whole batch (lengths, max_q, max_kv); equal calls give equal bits.  Limits: total_q * Hq * 2 +
  * B * num_heads * 512 under 2^32, B * (max_kv / 32 + 16) at most 2^30. */

@@ -53,13 +53,19 @@ template <int ROWB, bool CODES> __device__ __forceinline__ int v_swizzle(int row
   else return ((row >> 3) & 1) << 1;
 }
 
+// Weights of a second product in f16 (TV) are formed 2^14 over their share of the largest, which the sum and the result's quotient
+// carry alike: f16 keeps 11 bits down to 2^-28 of the largest weight and something down to 2^-39, where weights of at most 1 lose
+// bits from 2^-14 and become nothing at 2^-25.  (4999 keys 17.4 under one other hold 1.4e-4 of the probability, and all of the result in
+// columns where that one's value is zero; it came out as nothing there.)
+template <class TV> constexpr float weight_lift() { return std::is_same<TV, F16>::value ? 14.0f : 0.f; }
+
 // With codes the second product is in f16, in which they are exact, over the weights w = p vs (vs: V's scale of the key).  They are
-// formed as 2^(x + log2 vs - m), x the score's exponent and m the running maximum of these sums, so that w <= 1 has f16's range and
+// formed as 2^(x + log2 vs - m + 14), x the score's exponent and m the running maximum of x + log2 vs, so that w has f16's range and
 // 11 bits whatever the scales; the softmax's sum is that of w / vs, under the same m.  log2 vs and 1 / vs are formed once a key.
 // Error of the f32 result, 4000 keys, bf16 and f16 programs: 1.6e-4 (a product in bf16: 1.7e-3, and 4 to 8 % less time where
-// LDS waits show: 8 sequences of 1000 int8 keys 15.8 us, 15.2 so; at large batches level).  A scale under 1e-30 counts as
-// 1e-30: its row is nothing either way, and the key's probability has to come back from w / vs.
-__device__ __forceinline__ float weight_scale(float vs) { return fmaxf(vs, 1e-30f) + vs * 0.f; }      // (not finite: stays so)
+// LDS waits show: 8 sequences of 1000 int8 keys 15.8 us, 15.2 so; at large batches level).  A scale under 1e-25 counts as
+// 1e-25: its row is nothing either way, the key's probability has to come back from w / vs, and 2^30 such keys' sum stays finite.
+__device__ __forceinline__ float weight_scale(float vs) { return fmaxf(vs, 1e-25f) + vs * 0.f; }      // (not finite: stays so)
 
 template <int FMT, int DP> struct FewGeom {
   static constexpr int ESZ = FMT == kStorage ? 2 : 1;
@@ -179,6 +185,7 @@ __global__ __launch_bounds__((FewGeom<FMT, DP>::THREADS), (DP <= 128 && NQ == 1 
   constexpr int KSTEPS = DP / 16, DT = DP / 32, ROWB = G::ROWB, TILE = G::TILE, LD = G::LD, CHUNKS = G::CHUNKS;
   constexpr bool CODES = FMT != kStorage;
   constexpr int TILE_LOADS = 2 * LD + (CODES ? 1 : 0);
+  constexpr float LIFT = weight_lift<TV>();
 
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -480,7 +487,7 @@ __global__ __launch_bounds__((FewGeom<FMT, DP>::THREADS), (DP <= 128 && NQ == 1 
         m_run[qt] = m_new;
       }
       // (a row that has met no visible key keeps the sentinel: reference 0, so masked entries give P = 0)
-      const float mc = m_new > 0.5f * FA_NEG ? m_new * cs : 0.f;
+      const float mc = m_new > 0.5f * FA_NEG ? fmaf(m_new, cs, -LIFT) : 0.f;
       float sum = 0.f;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
@@ -578,7 +585,7 @@ __global__ __launch_bounds__((FewGeom<FMT, DP>::THREADS), (DP <= 128 && NQ == 1 
       acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
       const int i = 32 * qt + il, tok = p.ratio.quotient(i), hq = h * p.ratio.value + i - tok * p.ratio.value;
       const long row = (long)(s.q0 + tok) * p.Hq + hq;
-      const float lse = lt == 0.f ? -INFINITY : (mt * cs + cap.base + __log2f(lt)) * 0.69314718055994530942f;
+      const float lse = lt == 0.f ? -INFINITY : (mt * cs + (cap.base - LIFT) + __log2f(lt)) * 0.69314718055994530942f;
       if (whole) {
         if (!finite4(acc) || lt == 0.f) flags[il] = 1;
         store_o4<T>(p, s.q0 + tok, hq, d, acc);

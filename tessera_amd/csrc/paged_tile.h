@@ -113,6 +113,7 @@ __global__ __launch_bounds__((TileGeom<DP, W>::THREADS), (DP > 128 ? 1 : 2)) voi
   using TV = typename std::conditional<FMT == kStorage, T, BF16>::type;
   constexpr bool CODES = FMT != kStorage;
   constexpr bool SPLIT = splits_p<T, FMT>();
+  constexpr float LIFT = weight_lift<TV>();
   constexpr int THREADS = G::THREADS, BQ = G::BQ, KT = FA_BKV / 32, KSTEPS = DP / 16;
   constexpr int DT = DP / 32, ROWB = DP * 2, CHUNKS = DP / 8, TILE = G::TILE;
   // pieces of 16 bytes from memory: 8 values, or 16 codes
@@ -406,7 +407,7 @@ __global__ __launch_bounds__((TileGeom<DP, W>::THREADS), (DP > 128 ? 1 : 2)) voi
       m_run = m_new;
     }
     // (a row that has met no visible key yet keeps the sentinel: reference 0, its masked entries underflow to P = 0)
-    const float mc = m_new > 0.5f * FA_NEG ? m_new * cs : 0.f;
+    const float mc = m_new > 0.5f * FA_NEG ? fmaf(m_new, cs, -LIFT) : 0.f;
     constexpr int NU = 2 * KT, AHEAD = SPLIT ? 1 : 3;      // (units of P held before their product)
     uint4 pf[NU], pl[NU];
     float sum[2] = {0.f, 0.f};
@@ -520,7 +521,7 @@ __global__ __launch_bounds__((TileGeom<DP, W>::THREADS), (DP > 128 ? 1 : 2)) voi
   if (lh == 0 && rw + l32 < rows) {
     int tok, hq;
     row_of(rw + l32, tok, hq);
-    const float lse = l == 0.f ? -INFINITY : (m_run * cs + cap.base + __log2f(l)) * 0.69314718055994530942f;
+    const float lse = l == 0.f ? -INFINITY : (m_run * cs + (cap.base - LIFT) + __log2f(l)) * 0.69314718055994530942f;
     const long at_row = (long)(s.q0 + tok) * late.p.Hq + hq;
     if (!whole) late.part_lse[split * total_rows + at_row] = lse;
     else if (late.p.LSE) late.p.LSE[at_row] = lse;
