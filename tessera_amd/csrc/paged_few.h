@@ -186,6 +186,10 @@ __global__ __launch_bounds__((FewGeom<FMT, DP>::THREADS), (DP <= 128 && NQ == 1 
   constexpr bool CODES = FMT != kStorage;
   constexpr int TILE_LOADS = 2 * LD + (CODES ? 1 : 0);
   constexpr float LIFT = weight_lift<TV>();
+  // A far cap's exponents can be large and yet exact (every score of a row at the cap): log2 vs joins them behind the maximum, not rounded
+  // to their magnitude.  Elsewhere an exponent is as large as its score, whose f32 sum is off by more than that rounding, and the
+  // second read of log2 vs would cost 2 to 5 % (four tokens on 131072 int8 keys 65.9 -> 68.3 us).
+  constexpr bool LATE = CODES && FAR;
 
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -457,7 +461,7 @@ __global__ __launch_bounds__((FewGeom<FMT, DP>::THREADS), (DP <= 128 && NQ == 1 
           for (int r = 0; r < 16; ++r) sc[qt][r] *= c;
         }
       }
-      if constexpr (CODES) {
+      if constexpr (CODES && !LATE) {
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
           const float4 x = *reinterpret_cast<const float4*>(scales + 32 + 8 * a + 4 * lh);
@@ -469,12 +473,23 @@ __global__ __launch_bounds__((FewGeom<FMT, DP>::THREADS), (DP <= 128 && NQ == 1 
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = kv0 + 8 * (r >> 2) + 4 * lh + (r & 3);
-          if (key > khi[qt] || key < klo[qt]) sc[qt][r] = FA_NEG;
+          if (key > khi[qt] || key < klo[qt]) sc[qt][r] = FA_NEG;                 // (LATE: log2 vs is nothing beside it)
         }
       }
-      float mx = max3_raw(sc[qt][0], sc[qt][1], sc[qt][2]);
+      float mx;
+      if constexpr (LATE) {
+        mx = FA_NEG;
 #pragma unroll
-      for (int r = 3; r < 16; r += 2) mx = (r + 1 < 16) ? max3_raw(mx, sc[qt][r], sc[qt][r + 1]) : fmaxf(mx, sc[qt][r]);
+        for (int a = 0; a < 4; ++a) {
+          const float4 x = *reinterpret_cast<const float4*>(scales + 32 + 8 * a + 4 * lh);
+          mx = max3_raw(mx, sc[qt][4 * a + 0] + x.x, sc[qt][4 * a + 1] + x.y);
+          mx = max3_raw(mx, sc[qt][4 * a + 2] + x.z, sc[qt][4 * a + 3] + x.w);
+        }
+      } else {
+        mx = max3_raw(sc[qt][0], sc[qt][1], sc[qt][2]);
+#pragma unroll
+        for (int r = 3; r < 16; r += 2) mx = (r + 1 < 16) ? max3_raw(mx, sc[qt][r], sc[qt][r + 1]) : fmaxf(mx, sc[qt][r]);
+      }
       mx = max_with_other_half(mx);
       const float m_new = fmaxf(m_run[qt], mx);
       if (__any(m_new > m_run[qt])) {
@@ -491,9 +506,17 @@ __global__ __launch_bounds__((FewGeom<FMT, DP>::THREADS), (DP <= 128 && NQ == 1 
       float sum = 0.f;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
+        if constexpr (LATE) {
+#pragma unroll
+          for (int a = 2 * g; a < 2 * g + 2; ++a) {
+            const float4 x = *reinterpret_cast<const float4*>(scales + 32 + 8 * a + 4 * lh);
+            sc[qt][4 * a + 0] = sc[qt][4 * a + 0] - mc + x.x; sc[qt][4 * a + 1] = sc[qt][4 * a + 1] - mc + x.y;
+            sc[qt][4 * a + 2] = sc[qt][4 * a + 2] - mc + x.z; sc[qt][4 * a + 3] = sc[qt][4 * a + 3] - mc + x.w;
+          }
+        }
 #pragma unroll
         for (int r = 8 * g; r < 8 * g + 8; ++r) {
-          const float e = fast_exp2(CODES ? sc[qt][r] - mc : fmaf(sc[qt][r], cs, -mc));
+          const float e = fast_exp2(LATE ? sc[qt][r] : CODES ? sc[qt][r] - mc : fmaf(sc[qt][r], cs, -mc));
           sc[qt][r] = e;
           if (!CODES) sum += e;
         }

@@ -113,3 +113,43 @@ def test_a_long_flat_tail_under_one_key(lane, fmt, dtype, new, kv):
     hold(o, lse, ref, c, hq, new, slots)
     if fmt != "storage" and few_rows(c, hq, new) or fmt == "storage" and dtype == "f16":
         assert np.all(np.abs(o[..., ::2] - ref[0][..., ::2]) <= 2.0 ** -7 * np.abs(ref[0][..., ::2]) + 1e-30)
+
+
+@pytest.mark.parametrize("scale", (-0.3, 0.0, 1e-7, 2.0))
+@pytest.mark.parametrize("fmt,dtype", FORMATS)
+@pytest.mark.parametrize("new,kv", [([1, 2], [70, 300]), ([1], [3000]), ([100], [180])])
+def test_any_finite_scale_over_every_format(lane, scale, fmt, dtype, new, kv):
+    c, table, slots, q = make(lane, new, kv, hq=4, hkv=2, D=64, page=16, fmt=fmt, dtype=dtype, seed=34)
+    o, lse = attend(lane, c, table, q, new, kv, 4, scale=scale)
+    hold(o, lse, reference(c, slots, q, new, kv, 4, scale=scale), c, 4, new, slots)
+
+
+@pytest.mark.parametrize("fmt", ("storage", "i8", "e4m3"))
+@pytest.mark.parametrize("softcap", (0.0, 20.0, 1e6))
+@pytest.mark.parametrize("new,kv", [([1, 1], [100, 0]), ([1], [5000]), ([2] * 5, [900] * 5), ([60, 1], [200, 3]), ([50], [6000])])
+def test_scores_under_any_sentinel_over_every_format(lane, fmt, softcap, new, kv):
+    """Every visible score is near -8e32, or at the cap's lower end: finite and equal, so a row is the mean of the values it sees."""
+    c, table, slots, q = make(lane, new, kv, hq=4, hkv=2, D=64, page=16, fmt=fmt, dtype="bf16", seed=35)
+    q = to_bits(np.full(q.shape, 1e15), "bf16")
+    for s in slots:
+        at = (s // 16, s % 16)
+        if fmt == "storage":
+            c.k[at] = to_bits(np.float32(-1e17), "bf16")
+        else:
+            codes, scales = orc.kv_quantise(np.full((1, 64), -1e17, np.float32), fmt)
+            c.k[at], c.ks[at] = codes.view(np.uint8)[0], scales[0]
+    o, lse = attend(lane, c, table, q, new, kv, 4, softcap=softcap)
+    first, unit = 0, 2.0 ** -8
+    for b, n in enumerate(new):
+        keys, values = c.values(slots[b])
+        for i in range(n):
+            lo, hi = orc.key_bounds(i, n, kv[b], True, 0)
+            if hi < lo:
+                assert not o[first + i].any() and np.all(lse[first + i] == -np.inf)
+                continue
+            score = float(keys[lo, 0].sum()) * float(from_bits(q[:1, 0, 0], "bf16")[0]) * 64 ** -0.5
+            want = max(score, -softcap) if softcap else score
+            seen = values[lo:hi + 1].repeat(2, axis=1)
+            assert np.all(np.abs(o[first + i] - seen.mean(0)) <= (unit + (len(seen) + 4) * 2.0 ** -24) * np.abs(seen).mean(0) + 1e-7)
+            assert np.all(np.abs(lse[first + i] - want - (np.log(len(seen)) if softcap else 0)) <= 64 * 2.0 ** -24 * abs(want) + 1e-4)
+        first += n
