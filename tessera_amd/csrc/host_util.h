@@ -120,6 +120,9 @@ void* stream_workspace_or_null(hipStream_t s, size_t bytes);
 // At least `count` counters of a (device, stream) that are zero between calls: a kernel that counts in them leaves them
 // zero.  Kept and grown as the workspace is, in memory of their own.
 int* stream_counters(hipStream_t s, size_t count);
+// Outside of a capture grows a stream's workspace to `want` bytes (where that fails, to `need`) and its counters to `count`, for calls that a
+// capture may record later; inside one changes nothing.  Returns the bytes of workspace that are there.
+size_t stream_reserve(hipStream_t s, size_t need, size_t want, size_t count);
 // Status inside the library: the path needs scratch it could not have, nothing was launched, another path serves.
 constexpr int kNoScratch = -1;
 // Synchronises `s` and frees its workspace; a later call on the stream allocates afresh.

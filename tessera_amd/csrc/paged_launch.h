@@ -1,6 +1,7 @@
 // Host side of the paged attention kernels, instantiated once for each storage type and cache format.
 #pragma once
 #include <algorithm>
+#include <cstdint>
 #include <mutex>
 #include "host_util.h"
 #include "paged_merge.h"
@@ -30,7 +31,7 @@ inline int lds_limit(const void* kern, int bytes) {
 // How one call's work is divided.
 struct PagedPlan {
   bool few = false, tile = false;
-  int few_rows = 0, groups = 0, ahead = 0;
+  int few_rows = 0;
   int waves = 8, block = 0, blocks = 0, tile_split = 1;
 };
 
@@ -86,15 +87,17 @@ int launch_tile_for(const PagedTileParams& tp, const PagedPlan& plan, hipStream_
   return launch_tile<T, FMT, 256, 4>(tp, plan.blocks, s);
 }
 
+constexpr int kTileSplits = 32;
+
 // Workgroup size (8 waves: 256 rows, 4: 128; at DP = 256 always 4) and key splits of the tile kernel: the least estimated
 // time in us over both and up to 32 splits.  What it weighs, with times at D 128, Hq 32, Hkv 8, causal, bf16 pages:
 // - a workgroup costs 7 (4 waves: 6) and 1.6 to 2.05 a 64-key tile, the more of the chip works the more; 4 waves 1.45 to 1.65, and
 //   2.3 with a second workgroup on the compute unit (not at DP = 256): 512 tokens on 512 keys 21.7 in 8 waves, 18.4 in 4; 2048 on
 //   2048, two sequences, 85 and 92;
-// - splits leave partials and a merge, 4 us and the bytes: 1024 tokens on 8192 keys 220 unsplit, 153 in two, 183 in three
+// - splits leave partials (of at most `room` rows) and a merge, 4 us and the bytes: 1024 tokens on 8192 keys 220 unsplit, 153 in two, 183 in three
 //   (a second turn of workgroups); 100 on 16384 342 to 414, 52 as planned; but 512 on 512 18.4, 22.3 in two.
 // Returns the estimate.
-inline double plan_tiles(const PagedParams& p, bool codes, double chunks, PagedPlan& plan) {
+inline double plan_tiles(const PagedParams& p, bool codes, double chunks, int64_t room, PagedPlan& plan) {
   const int D = p.c.D, ratio = p.ratio.value, H = p.c.heads;
   const int64_t max_rows = (int64_t)p.max_q * ratio, all_rows = (int64_t)p.total_q * ratio;
   const double width = (D <= 64 ? 0.63 : D <= 128 ? 1.0 : 2.2) * (codes ? 1.2 : 1.0);
@@ -109,7 +112,7 @@ inline double plan_tiles(const PagedParams& p, bool codes, double chunks, PagedP
     const int64_t most = std::min<int64_t>(p.B * ((max_rows + block - 1) / block), all_rows / block + p.B);
     // (chunks of one length, and single tokens where no other kernel has them)
     const double blocks = std::min<double>((double)most, chunks * std::ceil((double)max_rows / block) + (plan.few ? 0.0 : p.B - chunks));
-    for (int n = 1; n <= 32 && (n == 1 || n <= longest / 2); ++n) {
+    for (int n = 1; n <= kTileSplits && (n == 1 || (n <= longest / 2 && n * (int64_t)p.total_q * p.Hq <= room)); ++n) {
       const double wgs = blocks * H * n;
       const double load = std::min(1.0, wgs / 256);
       double t;
@@ -133,7 +136,7 @@ inline double plan_tiles(const PagedParams& p, bool codes, double chunks, PagedP
   return best;
 }
 
-inline PagedPlan paged_plan(const PagedParams& p, bool codes) {
+inline PagedPlan paged_plan(const PagedParams& p, bool codes, int64_t room) {
   PagedPlan plan;
   const int D = p.c.D, ratio = p.ratio.value, limit = paged_few_limit(D);
   const int64_t max_rows = (int64_t)p.max_q * ratio;
@@ -146,7 +149,7 @@ inline PagedPlan paged_plan(const PagedParams& p, bool codes) {
   // Sequences that are chunks, as far as the host can tell: of the longest length, the others of one token.
   const double chunks = std::min<double>(p.B, std::max(1.0, std::ceil((double)(p.total_q - p.B) / std::max(p.max_q - 1, 1))));
   PagedPlan both = plan;
-  const double all = plan_tiles(p, codes, chunks, plan);
+  const double all = plan_tiles(p, codes, chunks, room, plan);
   // Single tokens beside chunks: the few-rows kernel takes the sequences with up to a tile's rows (or a token's, where the
   // group is larger), where its launch (10 us) and its reads cost less than such sequences among the tiles: 31 of 3000 to
   // 6000 keys beside a chunk of 500 tokens, e4m3, yes; 4 of 464 keys beside one of 202, no.
@@ -155,46 +158,79 @@ inline PagedPlan paged_plan(const PagedParams& p, bool codes) {
     both.few = true;
     both.few_rows = single;
     const double reads = 2.0 * (p.B - chunks) * p.c.heads * paged_span(p, 1) * D * (codes ? 1 : 2);
-    if (plan_tiles(p, codes, chunks, both) + 10 + reads / 5e6 < all) return both;
+    if (plan_tiles(p, codes, chunks, room, both) + 10 + reads / 5e6 < all) return both;
   }
   return plan;
 }
 
+// Rows of partials that no call needs more of whose arguments are no larger: every eager call makes room for them, so that
+// a capture behind it finds what the recorded call needs, whichever plan that one has.  Few rows: as many groups as the LDS lets
+// a compute unit hold, of the most rows (plan_few).  Split walks: 2^17 rows (68 MB at D 128; 512 tokens of 32 heads in eight parts);
+// where a recorded call's plan has more of them than there is room for, it is made again with fewer splits.
+template <int FMT>
+size_t few_reserve(const PagedParams& p) {
+  const int D = p.c.D, smem = D <= 64 ? FewGeom<FMT, 64>::SMEM : D <= 128 ? FewGeom<FMT, 128>::SMEM : FewGeom<FMT, 256>::SMEM;
+  const int waves = D <= 64 ? FewGeom<FMT, 64>::WAVES : D <= 128 ? FewGeom<FMT, 128>::WAVES : FewGeom<FMT, 256>::WAVES;
+  const int64_t tiles = (int64_t)p.B * ceil_div(p.max_kv, 32), groups = std::max<int64_t>(p.B, tiles / (2 * waves));
+  const int64_t rows = std::min<int64_t>(paged_few_limit(D), (int64_t)p.max_q * p.ratio.value);
+  return (size_t)(std::min<int64_t>(256 * (160 * 1024 / smem), groups * p.c.heads) * 2 * rows);
+}
+inline size_t tile_reserve(const PagedParams& p) {
+  if ((int64_t)p.max_q * p.ratio.value <= paged_few_limit(p.c.D)) return 0;
+  return (size_t)std::min<int64_t>((int64_t)kTileSplits * p.total_q * p.Hq, 1 << 17);
+}
+
+// The few-rows part of a plan: its kernel and how the axis is cut.
+template <class T, int FMT>
+bool plan_few(const PagedPlan& plan, PagedFewParams& fp, FewKernel& few) {
+  const PagedParams& p = fp.p;
+  few = few_kernel_for<T, FMT>(p, plan.few_rows);
+  if (few.per_cu <= 0) return false;
+  // As many equal shares as the chip holds workgroups for every head, at least one for a sequence and two tiles
+  // for a wave.  Starting a sequence costs about two steps of a workgroup.
+  const int waves = few.threads / 64;
+  const int64_t tiles = (int64_t)p.B * paged_tiles(p, plan.tile ? ceil_div(plan.few_rows, p.ratio.value) : p.max_q, 32);
+  fp.rows = plan.few_rows;
+  fp.ahead = p.B > 1 ? 2 * waves : 0;
+  fp.groups = (int)std::max<int64_t>(1, std::min<int64_t>(256 * few.per_cu / p.c.heads, std::max<int64_t>(p.B, tiles / (2 * waves))));
+  // Nothing is cut where a sequence takes two steps, or eight where the workgroups fill half of the chip anyway.
+  const int64_t each = tiles / p.B;
+  if (each <= 2 * waves || (each <= 8 * waves && (int64_t)p.B * p.c.heads >= 128 * few.per_cu)) fp.groups = 0;
+  // (the rule of the contiguous decode kernel, common.h)
+  fp.once = 64.0 * tiles * p.c.heads * p.c.D * (FMT == kStorage ? 2 : 1) >= kStreamOnceBytes;
+  return true;
+}
+
 template <class T, int FMT>
 int launch_paged(const PagedParams& p, hipStream_t s) {
-  const PagedPlan plan = paged_plan(p, FMT != kStorage);
+  const size_t D = (size_t)p.c.D, row_bytes = (D + 1) * sizeof(float);
   PagedFewParams fp{};
   PagedTileParams tp{};
   fp.p = p;
   tp.p = p;
+  FewKernel few{};
+  PagedPlan plan;
+  size_t fr = 0, tr = 0;                                   // rows of partials
+  auto make_plan = [&](int64_t room) {
+    plan = paged_plan(p, FMT != kStorage, room);
+    fp.groups = 0;
+    if (plan.few && !plan_few<T, FMT>(plan, fp, few)) return false;
+    fr = fp.groups > 1 ? (size_t)fp.groups * p.c.heads * 2 * fp.rows : 0;
+    tr = plan.tile && plan.tile_split > 1 ? (size_t)plan.tile_split * p.total_q * p.Hq : 0;
+    return true;
+  };
+  if (!make_plan(INT64_MAX)) return kDeviceFailed;
+  const size_t most = few_reserve<FMT>(p) + tile_reserve(p);
+  const size_t there = stream_reserve(s, (fr + tr) * row_bytes, std::max(fr + tr, most) * row_bytes, (size_t)p.B * p.c.heads) / row_bytes;
+  if (tr && fr + tr > there && !make_plan((int64_t)there - (int64_t)few_reserve<FMT>(p))) return kDeviceFailed;
   tp.nsplit = plan.tile_split;
   tp.min_rows = plan.few_rows;
-  FewKernel few{};
-  if (plan.few) {
-    few = few_kernel_for<T, FMT>(p, plan.few_rows);
-    if (few.per_cu <= 0) return kDeviceFailed;
-    // As many equal shares as the chip holds workgroups for every head, at least one for a sequence and two tiles
-    // for a wave.  Starting a sequence costs about two steps of a workgroup.
-    const int waves = few.threads / 64;
-    const int64_t tiles = (int64_t)p.B * paged_tiles(p, plan.tile ? ceil_div(plan.few_rows, p.ratio.value) : p.max_q, 32);
-    fp.rows = plan.few_rows;
-    fp.ahead = p.B > 1 ? 2 * waves : 0;
-    fp.groups = (int)std::max<int64_t>(1, std::min<int64_t>(256 * few.per_cu / p.c.heads, std::max<int64_t>(p.B, tiles / (2 * waves))));
-    // Nothing is cut where a sequence takes two steps, or eight where the workgroups fill half of the chip anyway.
-    const int64_t each = tiles / p.B;
-    if (each <= 2 * waves || (each <= 8 * waves && (int64_t)p.B * p.c.heads >= 128 * few.per_cu)) fp.groups = 0;
-    // (the rule of the contiguous decode kernel, common.h)
-    fp.once = 64.0 * tiles * p.c.heads * p.c.D * (FMT == kStorage ? 2 : 1) >= kStreamOnceBytes;
-  }
   const bool few_cut = fp.groups > 1, tile_cut = plan.tile && plan.tile_split > 1;
   // A sequence's partials are merged by the last of its workgroups, or by a kernel of their own: more than 16 of them, or
   // more than two passes of a workgroup's threads of a few sequences.
   const bool few_kernel_merges = few_cut && (fp.groups > 16 * p.B || (p.B <= 16 && fp.rows * p.c.D / 4 > 2 * few.threads));
   if (few_cut || tile_cut) {
-    const size_t D = (size_t)p.c.D;
-    const size_t fr = few_cut ? (size_t)fp.groups * p.c.heads * 2 * fp.rows : 0;
-    const size_t tr = tile_cut ? (size_t)plan.tile_split * p.total_q * p.Hq : 0;
-    float* ws = static_cast<float*>(stream_workspace(s, (fr + tr) * (D + 1) * sizeof(float)));
+    float* ws = static_cast<float*>(stream_workspace(s, (fr + tr) * row_bytes));
     if (!ws) return kDeviceFailed;
     fp.part_o = ws;
     tp.part_o = ws + fr * D;
@@ -217,7 +253,6 @@ int launch_paged(const PagedParams& p, hipStream_t s) {
   }
   if (!tile_cut) return kOk;
   const dim3 grid((unsigned)(plan.blocks * p.c.heads), (unsigned)(plan.block / 32));
-  const int D = p.c.D;
   auto merge = D <= 64 ? paged_tile_merge_kernel<T, FMT, 64> : D <= 128 ? paged_tile_merge_kernel<T, FMT, 128> : paged_tile_merge_kernel<T, FMT, 256>;
   hipLaunchKernelGGL(merge, grid, dim3(256), 0, s, tp, plan.block);
   return launch_status();

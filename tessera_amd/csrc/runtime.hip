@@ -76,6 +76,7 @@ struct WorkspaceSlot {
   std::vector<void*> retired;      // outgrown buffers: work queued before the growth may still use them
   int* counters = nullptr;         // zero between calls
   size_t count = 0;
+  size_t refused = 0;              // bytes that stream_reserve could not have, not asked for again; 0: none
 };
 std::mutex g_ws_mu;
 std::map<std::pair<int, hipStream_t>, WorkspaceSlot> g_ws_slots;
@@ -120,6 +121,35 @@ int* stream_counters(hipStream_t s, size_t count) {
   slot.counters = static_cast<int*>(p);
   slot.count = want;
   return slot.counters;
+}
+
+size_t stream_reserve(hipStream_t s, size_t need, size_t want, size_t count) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) { (void)hipGetLastError(); return 0; }
+  size_t bytes = 0, counters = 0, refused = 0;
+  auto look = [&] {
+    std::lock_guard<std::mutex> lock(g_ws_mu);
+    auto it = g_ws_slots.find({dev, s});
+    if (it == g_ws_slots.end()) return;
+    bytes = it->second.bytes;
+    counters = it->second.count;
+    refused = it->second.refused;
+  };
+  look();
+  if (refused != 0 && want >= refused) want = need;
+  if (bytes >= want && counters >= count) return bytes;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(s, &status) != hipSuccess) (void)hipGetLastError();
+  if (status != hipStreamCaptureStatusNone) return bytes;
+  if (bytes < want && !stream_workspace(s, want)) {
+    std::unique_lock<std::mutex> lock(g_ws_mu);
+    g_ws_slots[{dev, s}].refused = want;
+    lock.unlock();
+    if (bytes < need) (void)stream_workspace(s, need);
+  }
+  if (counters < count) (void)stream_counters(s, count);
+  look();
+  return bytes;
 }
 
 void* stream_workspace_or_null(hipStream_t s, size_t bytes) {
