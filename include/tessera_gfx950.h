@@ -54,13 +54,16 @@
  * router logits it uses no memory of the library's and has neither restriction (given a router
  * weight, the router product is a GEMM like any other and may split K through the stream's
  * workspace).  Calls that need the workspace: 8-bit products that split K on tiles (tile_m 128 or 256 by the query below),
- * attention that splits the keys (decode, and prefill with under 192 blocks of 256 query rows), paged attention (whose arrival
- * counters, zero between calls, are the stream's as its workspace is), routing,
- * combine and quantiser calls; recorded without one that is large enough they fail.  Three kinds use it where it
+ * attention that splits the keys (decode, and prefill with under 192 blocks of 256 query rows), paged attention that divides few
+ * rows (whose arrival counters, zero between calls, are the stream's as its workspace is), routing,
+ * combine and quantiser calls; recorded without one that is large enough they fail.  (Whether a paged call needs any, and how much, does
+ * not grow with its arguments alone, so an eager one makes room for every call whose B, total_q, max_q and max_kv are no larger over
+ * the same heads and head dimension: 2 to 70 MB, with chunks 70 to 140 more.)  Four kinds use it where it
  * is there and large enough and take a path without it inside a capture where it is not, on a stream that has run
  * nothing eagerly as on one whose eager calls were smaller: single 16-bit products, single 8-bit products on the streaming kernel
- * (up to 64 rows, tile_m 32 or 64), and attention of few query rows at head dimensions other than 64, 128 and 256 with 192 and
- * more (batch, head) pairs or under 1024 keys.  The products then keep K whole: the f32 sums are added in another order
+ * (up to 64 rows, tile_m 32 or 64), attention of few query rows at head dimensions other than 64, 128 and 256 with 192 and
+ * more (batch, head) pairs or under 1024 keys, and paged chunks whose key walk is split (recorded in as many parts as there is room
+ * for, which behind an eager call as large is 2^17 rows of partials at least).  The products then keep K whole: the f32 sums are added in another order
  * than the eager call's, and few rows or few tiles under a long K take up to six times as long (64 x 896 x 14000: 82 us for
  * 14).  Nothing reports it; the eager call with arguments as large avoids it.  Any entry point
  * (tessera_gfx950_probe is the cheapest) must have been called once before the first capture: the first call initialises the device.
