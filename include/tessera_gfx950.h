@@ -517,7 +517,8 @@ int tessera_gfx950_kv_cache_read_bf16_dev(const tessera_gfx950_kv_cache* cache, 
  * boundaries; Hq a multiple of num_heads, KV head = hq / (Hq / num_heads); LSE f32 [total_q, Hq] or NULL; out_dtype 0 = f32
  * O, 1 = the storage type.  max_q and max_kv: no sequence has more new tokens or more keys (a longer one is cut to
  * them), max_kv <= pages_per_seq * page_size.  Device values out of their range are held to it: a wrong offset, length or
- * page gives wrong rows and no access outside of the arrays.
+ * page gives wrong rows and no access outside of the arrays.  Rows of Q past q_offsets[B] and those of sequences that max_q cuts are not
+ * attended: their rows of O and LSE are left as they are.
  *
  * Scores, softmax statistics and sums are f32.  A probability is rounded once before the second product, to the storage type; over
  * 8-bit formats the second product's weights, probability times scale, have 11 bits where a sequence has few rows, else 8, and 16 in

@@ -129,8 +129,10 @@ class PagedKVCache:
 @dataclass
 class PagedBatch:
     """One call's sequences: their new tokens are rows ``q_offsets[b] .. q_offsets[b + 1]`` of Q, their keys (the new ones
-    among them) ``kv_lens[b]`` slots through ``page_table[b]``; ``slots`` are the new tokens' own."""
-    slots: DeviceArray          # i64 [T]
+    among them) ``kv_lens[b]`` slots through ``page_table[b]``; ``slots`` are the new tokens' own.  A Q has as many rows as there
+    are slots; a batch of fewer rows than were written (the last token of each sequence, say) leaves the slots out.  Rows that
+    no sequence has (where slots outside of the cache fill a batch up) are not written."""
+    slots: Optional[DeviceArray]    # i64 [T]
     page_table: DeviceArray     # i32 [B, pages]
     q_offsets: DeviceArray      # i32 [B + 1]
     kv_lens: DeviceArray        # i32 [B]
@@ -199,6 +201,8 @@ def _attend(q_ptr: int, q_token: int, T: int, Hq: int, cache: PagedKVCache, batc
     if any(a.dtype != "i32" for a in (table, offsets, lens)) or table.ndim != 2:
         raise ValueError("page_table, q_offsets and kv_lens must be i32, page_table (B, pages)")
     B, D = table.shape[0], cache.head_dim
+    if batch.slots is not None and batch.slots.shape != (T,):
+        raise ValueError(f"queries of {T} tokens for a batch of {batch.slots.shape[0]}")
     if offsets.shape != (B + 1,) or lens.shape != (B,):
         raise ValueError(f"q_offsets {offsets.shape} and kv_lens {lens.shape} for {B} sequences")
     O = _result((T, Hq, D), "f32" if out == "f32" else cache.dtype)

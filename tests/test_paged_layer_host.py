@@ -1,0 +1,65 @@
+"""No-GPU checks of the paged cache's Python layer and of what a cache that is written has to look like."""
+import ctypes
+from types import SimpleNamespace
+
+import numpy as np
+import pytest
+
+from tessera_amd import lane, paged
+from test_paged_host import attend, handle, read, write
+
+
+class Host:
+    """Stands in for a device array."""
+    fail_at = None
+    made = 0
+
+    def __init__(self, a):
+        self.a, self.shape, self.ndim, self.address = a, a.shape, a.ndim, 1 << 24
+        self.dtype = {"int64": "i64", "int32": "i32", "float16": "f16"}[a.dtype.name]
+
+    @classmethod
+    def from_host(cls, a):
+        cls.made += 1
+        if cls.made == cls.fail_at:
+            raise RuntimeError("malloc: device operation failed")
+        return cls(np.ascontiguousarray(a))
+
+
+@pytest.fixture
+def host(monkeypatch):
+    monkeypatch.setattr(paged, "DeviceArray", Host)
+    monkeypatch.setattr(Host, "fail_at", None)
+    monkeypatch.setattr(Host, "made", 0)
+    return Host
+
+
+def small(**change):
+    return SimpleNamespace(**{**dict(num_pages=6, page_size=4, num_kv_heads=2, head_dim=64, dtype="f16", handle=handle()), **change})
+
+
+@pytest.mark.parametrize("tokens", (2, 4))
+def test_queries_and_batch_have_as_many_tokens(host, monkeypatch, tokens):
+    """Rows of O behind the batch's tokens would be an earlier result's memory, rows that are not there the last sequences'."""
+    monkeypatch.setattr(paged, "_result", lambda shape, dtype: pytest.fail("a result was made"))
+    cache = small()
+    batch = paged.SequencePages(cache).extend({"a": 2, "b": 1})
+    with pytest.raises(ValueError, match="3"):
+        paged.paged_attention(Host(np.zeros((tokens, 4, 64), np.float16)), cache, batch)
+    with pytest.raises(ValueError, match="3"):
+        paged.paged_attention_fused_qkv(Host(np.zeros((tokens, 8 * 64), np.float16)), 4, cache, batch)
+
+
+def test_a_batch_without_slots_is_not_compared(host, monkeypatch):
+    """A caller's own batch of fewer rows than were written (the last token of each sequence) leaves the slots out."""
+    class Reached(Exception):
+        pass
+
+    def result(shape, dtype):
+        raise Reached
+    monkeypatch.setattr(paged, "_result", result)
+    cache = small()
+    step = paged.SequencePages(cache).extend({"a": 2, "b": 1})
+    last = paged.PagedBatch(None, step.page_table, Host(np.asarray([0, 1, 2], np.int32)), step.kv_lens, 1, 2)
+    with pytest.raises(Reached):
+        paged.paged_attention(Host(np.zeros((2, 4, 64), np.float16)), cache, last)
