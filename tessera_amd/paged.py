@@ -169,7 +169,7 @@ class SequencePages:
 
     def extend(self, new_tokens: Dict[Hashable, int]) -> PagedBatch:
         """Room for ``new_tokens[seq]`` more tokens of each sequence (new ones start empty), and the batch's arrays.
-        ``MemoryError`` where the cache has too few free pages; nothing is taken then."""
+        ``MemoryError`` where the cache has too few free pages; nothing is taken then, nor where the arrays cannot be made."""
         size = self.cache.page_size
         if any(n < 0 for n in new_tokens.values()):
             raise ValueError("a sequence cannot lose tokens")
@@ -177,9 +177,22 @@ class SequencePages:
         if sum(want.values()) > len(self._free):
             raise MemoryError(f"{sum(want.values())} pages wanted, {len(self._free)} free")
         before = {s: self.length(s) for s in new_tokens}
+        known = {s for s in new_tokens if s in self._pages}
         for s, n in new_tokens.items():
             self._pages.setdefault(s, []).extend(self._free.pop() for _ in range(want[s]))
             self._length[s] = before[s] + n
+        try:
+            return self._batch(new_tokens, before)
+        except BaseException:                                  # (no arrays, no step: the pages go back in the order they came)
+            for s in reversed(list(new_tokens)):
+                for _ in range(want[s]):
+                    self._free.append(self._pages[s].pop())
+                self._length[s] = before[s]
+                if s not in known:
+                    del self._pages[s], self._length[s]
+            raise
+
+    def _batch(self, new_tokens: Dict[Hashable, int], before: Dict[Hashable, int]) -> PagedBatch:
         seqs = list(new_tokens)
         width = max([len(self._pages[s]) for s in seqs] + [1])
         table = np.zeros((len(seqs), width), np.int32)

@@ -63,3 +63,17 @@ def test_a_batch_without_slots_is_not_compared(host, monkeypatch):
     last = paged.PagedBatch(None, step.page_table, Host(np.asarray([0, 1, 2], np.int32)), step.kv_lens, 1, 2)
     with pytest.raises(Reached):
         paged.paged_attention(Host(np.zeros((2, 4, 64), np.float16)), cache, last)
+
+
+@pytest.mark.parametrize("at", (1, 2, 3, 4))
+def test_a_step_whose_arrays_cannot_be_made_takes_nothing(host, at):
+    pages = paged.SequencePages(small())
+    pages.extend({"a": 3})
+    before = (pages.free_pages, list(pages._free), pages.slots("a").tolist(), pages.length("a"), pages.length("b"))
+    host.fail_at = host.made + at
+    with pytest.raises(RuntimeError):
+        pages.extend({"a": 9, "b": 2, "c": 0})
+    assert (pages.free_pages, list(pages._free), pages.slots("a").tolist(), pages.length("a"), pages.length("b")) == before
+    assert set(pages._pages) == {"a"} and set(pages._length) == {"a"}
+    batch = pages.extend({"a": 9, "b": 2})
+    assert pages.length("a") == 12 and pages.length("b") == 2 and len(set(batch.slots.a.tolist())) == 11
