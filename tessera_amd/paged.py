@@ -157,8 +157,12 @@ class SequencePages:
         return self._length.get(seq, 0)
 
     def slots(self, seq: Hashable, first: int = 0, last: Optional[int] = None) -> np.ndarray:
-        """Slot numbers of a sequence's tokens [first, last), as ``read`` takes them."""
-        at = np.arange(first, self.length(seq) if last is None else last, dtype=np.int64)
+        """Slot numbers of a sequence's tokens [first, last), as ``read`` takes them; ``IndexError`` past its end."""
+        end = self.length(seq)
+        last = end if last is None else last
+        if not 0 <= first <= last <= end:
+            raise IndexError(f"tokens [{first}, {last}) of a sequence of {end}")
+        at = np.arange(first, last, dtype=np.int64)
         pages = np.asarray(self._pages.get(seq, []), np.int64)
         return pages[at // self.cache.page_size] * self.cache.page_size + at % self.cache.page_size
 

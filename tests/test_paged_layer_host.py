@@ -77,3 +77,15 @@ def test_a_step_whose_arrays_cannot_be_made_takes_nothing(host, at):
     assert set(pages._pages) == {"a"} and set(pages._length) == {"a"}
     batch = pages.extend({"a": 9, "b": 2})
     assert pages.length("a") == 12 and pages.length("b") == 2 and len(set(batch.slots.a.tolist())) == 11
+
+
+def test_slots_are_those_of_tokens_that_are_there(host):
+    """Beyond a sequence's end lie slots of its last page that hold nothing of it."""
+    pages = paged.SequencePages(small())
+    pages.extend({"a": 5})
+    assert len(pages.slots("a")) == 5 and len(pages.slots("a", 2, 4)) == 2 and len(pages.slots("a", 5)) == 0 and len(pages.slots("nobody")) == 0
+    for first, last in ((0, 6), (0, 9), (-1, None), (6, None), (3, 2), (0, -1)):
+        with pytest.raises(IndexError):
+            pages.slots("a", first, last)
+    with pytest.raises(IndexError):
+        pages.slots("nobody", 0, 1)
