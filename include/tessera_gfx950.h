@@ -476,7 +476,8 @@ int tessera_gfx950_flash_attn_bias_bf16_dev(const void* Q, const void* K, const 
  *
  * Strides are element strides of (page, place, head), the last dimension is contiguous; [pages, page_size, heads, D] and
  * [pages, heads, page_size, D] are both served.  K, V and their strides lie on the 16-byte grid; a stride is under 2 GiB
- * (the cache itself may be larger), scale strides under 2^31.  All pointers are device
+ * (the cache itself may be larger), scale strides under 2^31.  A cache that is written has rows and scales that do not overlap: in the
+ * order of the strides, each is at least what the smaller ones span; one that is only read may share them.  All pointers are device
  * memory; the struct itself is host memory and is read during the call only. */
 typedef struct {
   void* k;

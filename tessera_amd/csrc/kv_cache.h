@@ -4,6 +4,7 @@
 // dimensions is served through strides.  Format kStorage holds 16-bit values; kInt8 and kE4m3 hold codes with one f32
 // scale for each (slot, head): value = code * scale.
 #pragma once
+#include <algorithm>
 #include <type_traits>
 #include "../../include/tessera_gfx950.h"
 #include "common.h"
@@ -69,7 +70,7 @@ inline KvCache device_view(const tessera_gfx950_kv_cache& c) {
 }
 
 // Whether a cache cannot be served: sizes, the 16-byte grid of rows and pointers (every row is moved 16 or 8 bytes at a
-// time), rows that would overlap, strides of 2 GiB and more (a page's and a slot's offsets are 32 by 32 bit products).  Slot
+// time), strides under a row (whether rows overlap otherwise matters to a write: rows_overlap), strides of 2 GiB and more (a page's and a slot's offsets are 32 by 32 bit products).  Slot
 // numbers fit 31 bits.
 inline bool bad_cache(const tessera_gfx950_kv_cache* c) {
   if (!c || !c->k || !c->v || c->format < kStorage || c->format > kE4m3) return true;
@@ -91,6 +92,26 @@ inline bool bad_cache(const tessera_gfx950_kv_cache* c) {
   for (int i = 0; i < 3; ++i)
     if (c->scale_strides[i] < 0 || c->scale_strides[i] > 0x7fffffff || (size[i] > 1 && c->scale_strides[i] < 1)) return true;
   return false;
+}
+
+// Whether rows of `width` elements share elements: taken by their strides, each has to be at least what the smaller ones span.  (Orders that
+// interleave without that, strides 2 and 3 of two each, are taken to overlap.)
+inline bool rows_overlap(const int64_t strides[3], const int size[3], int width) {
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + 3, [&](int a, int b) { return strides[a] < strides[b]; });
+  int64_t span = width;
+  for (int i : order) {
+    if (size[i] == 1) continue;
+    if (strides[i] < span) return true;
+    span += strides[i] * (size[i] - 1);                  // (under 2^31 before the last, 2^62 there)
+  }
+  return false;
+}
+// Whether a write to a cache that is not bad would put rows, or scales, on top of each other.
+inline bool overlapping_cache(const tessera_gfx950_kv_cache& c) {
+  const int size[3] = {c.num_pages, c.page_size, c.num_heads};
+  return rows_overlap(c.k_strides, size, c.head_dim) || rows_overlap(c.v_strides, size, c.head_dim) ||
+         (c.format != kStorage && rows_overlap(c.scale_strides, size, 1));
 }
 
 // Four codes (one dword) as f32.

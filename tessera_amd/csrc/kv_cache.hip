@@ -174,7 +174,7 @@ int launch_rows_for(bool write, const KvCache& c, const void* k, const void* v, 
 template <class T>
 int cache_rows(bool write, const tessera_gfx950_kv_cache* cache, const void* k, const void* v, const int64_t* strides,
                const int64_t* slots, int tokens, void* stream) {
-  if (bad_cache(cache) || tokens < 0) return kBadShape;
+  if (bad_cache(cache) || tokens < 0 || (write && overlapping_cache(*cache))) return kBadShape;
   if (tokens == 0) return probe_device();
   if (!slots || bad_rows(k, v, strides, cache->head_dim, tokens, cache->num_heads, !write)) return kBadShape;
   // (rows are 32-bit numbers, and so are a launch's threads, up to 32 for a row)

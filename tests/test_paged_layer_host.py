@@ -89,3 +89,32 @@ def test_slots_are_those_of_tokens_that_are_there(host):
             pages.slots("a", first, last)
     with pytest.raises(IndexError):
         pages.slots("nobody", 0, 1)
+
+
+CODES = dict(format=1, k_scale=1 << 22, v_scale=1 << 23)
+
+
+@pytest.mark.parametrize("change", [
+    dict(k_strides=(64, 64, 64)), dict(v_strides=(64, 64, 64)), dict(k_strides=(2048, 64, 64)), dict(v_strides=(1024, 128, 64)),
+    dict(k_strides=(64, 128, 1024)), dict(k_strides=(128, 128, 64), page_size=1, num_pages=4, num_heads=3),
+    dict(**CODES, scale_strides=(1, 1, 1)), dict(**CODES, scale_strides=(16, 2, 1)), dict(**CODES, k_strides=(1024, 128, 64))], ids=str)
+def test_rows_on_top_of_each_other_are_not_written(change):
+    """Two slots or heads of one cache in the same memory: what a write leaves there would depend on the order of its waves."""
+    assert write(handle(**change)) == lane.BAD_SHAPE
+
+
+@pytest.mark.parametrize("change", [
+    dict(), dict(k_strides=(2048, 64, 1024)), dict(k_strides=(128, 256, 64)), dict(v_strides=(64, 256, 128), k_strides=(4096, 256, 128)),
+    dict(num_pages=1, k_strides=(0, 128, 64)), dict(num_heads=1, k_strides=(1024, 64, 0)), dict(page_size=1, k_strides=(128, 8, 64)),
+    dict(**CODES), dict(**CODES, scale_strides=(1, 4, 2)), dict(**CODES, scale_strides=(64, 4, 1))], ids=str)
+def test_caches_of_any_order_and_with_gaps_are_written(change):
+    if lane.available():
+        pytest.skip("made-up addresses: only where there is no device to use them on")
+    c = handle(**change)
+    assert write(c) == read(c) == attend(c, max_kv=2, max_q=2, total=2) == lane.NO_DEVICE
+
+
+def test_caches_that_are_only_read_may_share_rows():
+    if lane.available():
+        pytest.skip("made-up addresses: only where there is no device to use them on")
+    assert read(handle(k_strides=(64, 64, 64))) == attend(handle(k_strides=(64, 64, 64))) == lane.NO_DEVICE
