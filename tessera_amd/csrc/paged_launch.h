@@ -248,7 +248,9 @@ int launch_paged(const PagedParams& p, hipStream_t s) {
     if (int rc = launch_status(); rc != kOk) return rc;
   }
   if (few_kernel_merges) {
-    hipLaunchKernelGGL((paged_few_merge_kernel<T, FMT>), dim3((unsigned)p.total_q, (unsigned)p.Hq), dim3(256), 0, s, fp);
+    // (a dimension's threads are a 32-bit number; what is beyond it wraps, without an error)
+    const unsigned tokens = (unsigned)p.total_q, along = std::min(tokens, 1u << 23);
+    hipLaunchKernelGGL((paged_few_merge_kernel<T, FMT>), dim3(along, (unsigned)p.Hq, (tokens + along - 1) / along), dim3(256), 0, s, fp);
     if (int rc = launch_status(); rc != kOk) return rc;
   }
   if (!tile_cut) return kOk;

@@ -95,7 +95,10 @@ __global__ __launch_bounds__(256) void paged_few_merge_kernel(const PagedFewPara
   __shared__ float sh_sum[256], sh_red[4];
   const PagedParams& p = fp.p;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, D = p.c.D;
-  const int t = blockIdx.x, hq = blockIdx.y;
+  const int hq = blockIdx.y;
+  const unsigned token = blockIdx.z * gridDim.x + blockIdx.x;
+  if (token >= (unsigned)p.total_q) return;
+  const int t = (int)token;
   // the row's sequence, where it lies on the axis, and the share
   int total = 0, b = -1, start = 0, places = 0;
   PagedSeq s{0, 0, 0};

@@ -144,3 +144,22 @@ def test_steps_without_a_token(lane, quant):
         assert np.all(np.abs(o.to_host() - 1) <= 2.0 ** -3)
         got = cache.read(DeviceArray.from_host(pages.slots("a")))[0].to_host()
         assert got.shape == (pages.length("a"), 2, 64) and np.all(np.abs(got - 1) <= 2.0 ** -3)
+
+
+def test_more_tokens_than_one_launch_has_rows(lane):
+    """A buffer of 2^24 and more rows of Q, of which the sequence has a few: the merge of its shares is launched over all of them."""
+    lib, D, kv, total = lane.load(), 16, 9000, (1 << 24) + 40
+    c, table, slots, q = make(lane, [2], [kv], hq=1, hkv=1, D=D, page=64, fmt="storage", dtype="bf16", seed=43)
+    handle = c.upload()
+    Q, O = lane.DeviceBuffer(total * D * 2), lane.DeviceBuffer(total * D * 2)
+    for first in (0, total - 2):                                # its rows at the buffer's start, and at its end
+        lane.check(lib.tessera_gfx950_memcpy_h2d(Q.ptr + first * D * 2, q.ctypes.data, q.nbytes), "memcpy_h2d")
+        bufs = [lane.DeviceBuffer.from_host(a) for a in (table, np.asarray([first, first + 2], np.int32), np.asarray([kv], np.int32))]
+        lane.check(lib.tessera_gfx950_paged_attention_bf16_dev(
+            ctypes.byref(handle), Q.ptr, O.ptr, None, i64((D, D) * 2), bufs[0].ptr, table.shape[1], bufs[1].ptr, bufs[2].ptr, 1, 1, total, 2, kv, D ** -0.5, 1, 0, 0.0, 1,
+            None), "paged_attention")
+        lane.synchronize()
+        got = np.empty((2, 1, D), np.uint16)
+        lane.check(lib.tessera_gfx950_memcpy_d2h(got.ctypes.data, O.ptr + first * D * 2, got.nbytes), "memcpy_d2h")
+        ref = reference(c, slots, q, [2], [kv], 1)
+        hold(from_bits(got, "bf16"), ref[1].astype(np.float32), ref, c, 1, kv=kv)
