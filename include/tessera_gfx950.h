@@ -523,8 +523,9 @@ int tessera_gfx950_kv_cache_read_bf16_dev(const tessera_gfx950_kv_cache* cache, 
  *
  * Scores, softmax statistics and sums are f32.  A probability is rounded once before the second product, to the storage type; over
  * 8-bit formats the second product's weights, probability times scale, have 11 bits where a sequence has few rows, else 8, and 16 in
- * f16 programs.  Weights of 11 bits (f16) keep them down to 2^-28 of a row's largest and are nothing under 2^-39 of it.  Keys that a token does not see
- * leave its row as it is whatever they hold, infinities and NaN among it.  How a sequence's keys are divided, and so the order of
+ * f16 programs.  Weights of 11 bits (f16) keep them down to 2^-28 of a row's largest and are nothing under 2^-39 of it.  Keys that a
+ * token does not see leave its row as it is whatever they hold, infinities and NaN among it; rows that see such a value take a hundred
+ * times as long and more (one wave forms each again by the plain definition).  How a sequence's keys are divided, and so the order of
  * the sums, depends on the whole batch (lengths, max_q, max_kv); equal calls give equal bits.  Limits: total_q * Hq * 2 +
  * B * num_heads * 512 under 2^32, B * (max_kv / 32 + 16) at most 2^30. */
 int tessera_gfx950_paged_attention_f16_dev(const tessera_gfx950_kv_cache* cache, const void* Q, void* O, float* LSE,

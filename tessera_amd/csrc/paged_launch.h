@@ -96,6 +96,7 @@ constexpr int kTileSplits = 32;
 //   2048, two sequences, 85 and 92;
 // - splits leave partials (of at most `room` rows) and a merge, 4 us and the bytes: 1024 tokens on 8192 keys 220 unsplit, 153 in two, 183 in three
 //   (a second turn of workgroups); 100 on 16384 342 to 414, 52 as planned; but 512 on 512 18.4, 22.3 in two.
+// - codes 1.2 times as long in both forms (4 waves, 512 tokens on 512 keys: 18.7 over 16 bits, e4m3 22.4, int8 23.2; f16 programs 24.8 and 26.1).
 // Returns the estimate.
 inline double plan_tiles(const PagedParams& p, bool codes, double chunks, int64_t room, PagedPlan& plan) {
   const int D = p.c.D, ratio = p.ratio.value, H = p.c.heads;
