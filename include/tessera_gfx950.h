@@ -511,7 +511,7 @@ int tessera_gfx950_kv_cache_read_bf16_dev(const tessera_gfx950_kv_cache* cache, 
  * int32 [B + 1], ascending from 0) and kv_lens[b] keys (device int32 [B]), its new tokens' own, written before, among
  * them; key j is place j % page_size of page page_table[b][j / page_size] (device int32 [B, pages_per_seq]; entries past a
  * sequence's last page are not read).  Token i of n sees what row i of n queries sees in tessera_gfx950_flash_attn_ext with
- * Sk = kv_lens[b]: causal, window and softcap have the meaning they have there.  A token that sees no key gives O = 0,
+ * Sk = kv_lens[b]: causal, window and softcap have the meaning they have there (softcap finite).  A token that sees no key gives O = 0,
  * LSE = -inf.
  *
  * Q [total_q, Hq, D] and O through 4 element strides (Q token, Q head, O token, O head; multiples of 8), on 16-byte
